@@ -355,17 +355,14 @@ def _nearest(y):
     return torch.round(y / step) * step
 
 
-def _blocks64(y, rounded=False):
-    """What the codes and scales [..., blocks] of y hold, in 64 bits. As with every other type the values are those before
-    the rounding to the output's type; where the rounding is all that an operator does (`rounded`), they are the codes.
-    A scale is a choice among powers of two: it has such a value only where the largest magnitude is an input's own."""
+def _blocks64(y):
+    """e4m3 values and scales [..., blocks] of y, both in 64 bits."""
     cols = y.shape[-1]
     b = torch.nn.functional.pad(y, (0, -cols % BLOCK)).unflatten(-1, (-1, BLOCK))
     amax = b.abs().amax(-1)
     f = torch.exp2(torch.ceil(torch.log2((amax / 448).clamp(min=2.0 ** -127))))
     f = torch.where(amax > 448 * f, f * 2, torch.where(amax <= 224 * f, f / 2, f)).clamp(min=2.0 ** -127)
-    q = b / f[..., None]
-    return (_nearest(q) if rounded else q).flatten(-2)[..., :cols], f
+    return _nearest(b / f[..., None]).flatten(-2)[..., :cols], f
 
 
 def _words64(f):
@@ -382,9 +379,7 @@ def exact(case, seed):
             y = y / (y.square().mean(-1, keepdim=True) + EPS).sqrt()
             y = y.unflatten(0, (c["vecs"], -1)) * s["scale1"].to(d).reshape(c["vecs"], 1, -1) + s["shift"].to(d).reshape(c["vecs"], 1, -1)
             y = y.flatten(0, 1)
-        if c["op"] == "adaln":
-            return _blocks64(y)[0], None
-        q, f = _blocks64(y, rounded=True)
+        q, f = _blocks64(y)
         return q, _words64(f)
     if c["op"] == "gemm":
         def whole(q, w):
@@ -402,9 +397,10 @@ def exact(case, seed):
         y = (y[..., :16] / (1 + torch.exp(-y[..., :16])) * y[..., 16:]).reshape(c["m"], -1)
         if c["tail"] == "swiglu":
             return y
-        return _blocks64(y)[0], None
+        q, f = _blocks64(y)
+        return q, _words64(f)
     if c["op"] == "kv_write":
-        cache = s["cache"].to(d)
+        cache, scale = s["cache"].to(d), s["scale"].to(d)
         for b in range(c["batch"]):
             n = c["tokens"] if s["lens"] is None else int(s["lens"][b])
             first = 0 if s["start"] is None else int(s["start"][b])
@@ -417,8 +413,10 @@ def exact(case, seed):
                 z = torch.view_as_complex(k[:, :, :c["rope"]].reshape(n, c["layers"], c["rope"], 64, 2).contiguous())
                 k[:, :, :c["rope"]] = torch.view_as_real(z * cs).flatten(-2)
             kv[:, :, 0] = k
-            cache[b, first:first + n] = _blocks64(kv)[0]
-        return cache, None
+            q, f = _blocks64(kv)
+            cache[b, first:first + n] = q
+            scale[b, :, :, :, first:first + n] = f[..., 0].permute(1, 2, 3, 0)
+        return cache, scale
     out = torch.zeros(s["q"].shape, dtype=d, device="cuda")
     for r in range(out.shape[0]):
         ks, vs = ([s["k"][r].to(d)], [s["v"][r].to(d)]) if c["self"] else ([], [])
