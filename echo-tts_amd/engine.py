@@ -238,6 +238,11 @@ class CFGPlan:
                 self.loop()
                 if use_graph:
                     g = torch.cuda.CUDAGraph()
+                    # torch makes the RNG tensors of all live graphs with the first one that meets the generator. The
+                    # samplers run in inference_mode: made there they are inference tensors, and no graph could be
+                    # captured outside the mode while this plan lives
+                    with torch.inference_mode(False):
+                        g.register_generator_state(torch.cuda.default_generators[torch.cuda.current_device()])
                     with torch.cuda.graph(g):
                         self.loop()
                     self.graph = g
