@@ -158,8 +158,9 @@ __device__ __forceinline__ void write_out4(const Args& a, const float (&v)[4], f
 // The exponents' reference is the maximum of the first tile, and stays: a later score above it only makes P larger than 1,
 // and fp32 sums and a bf16 P hold any power of two up to 2^127 with the same relative precision. So the loop has no
 // maximum, no rescaling and no branch around O (which the compiler turns into 64 moves a tile). If a query's sum passes
-// 2^60 (a score 2^60 above the first tile's, or not finite) or its first tile has only -inf, the workgroup walks its tiles once more with the running
-// maximum (SAFE); so it does at once where a segment is causal, whose first tile may show a query nothing.
+// 2^60 (a score 2^60 above the first tile's, or not finite), one of its sums in O 2^100 (large values at such a score; up to
+// 64 parts of it still add up in the join) or its first tile has only -inf, the workgroup walks its tiles once more with the
+// running maximum (SAFE); so it does at once where a segment is causal, whose first tile may show a query nothing.
 template <bool SPLIT>
 __global__ void __launch_bounds__(256, 2) attn_fp8_kernel(EchoAttnFp8Args arg, float* ws, int nsplit) {
   (void)arg;
@@ -397,8 +398,13 @@ __global__ void __launch_bounds__(256, 2) attn_fp8_kernel(EchoAttnFp8Args arg, f
   bool redo = any_causal != 0;
   if (!redo) {
     walk(std::false_type{});
+    float most = 0.f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = __builtin_elementwise_maximum(most, __builtin_fabsf(o[d][r]));
     if (lane == 0) again[w] = 0;
-    if (__any(!(l_run <= 0x1p60f) || m_run == -INFINITY) && lane == 0) again[w] = 1;
+    if (__any(!(l_run <= 0x1p60f) || m_run == -INFINITY || !(most <= 0x1p100f)) && lane == 0) again[w] = 1;
     __syncthreads();
     redo = uni(again[0] | again[1] | again[2] | again[3]) != 0;
     __syncthreads();

@@ -405,8 +405,9 @@ int echo_gemm_fp8(const EchoGemmFp8Args* args, void* stream);
  * e4m3 codes in blocks of one head's 128 (head h of token t at k + b ld_batch + t ld_tok + h ld_head, in elements)
  * and scale bytes at k_scale + b s_batch + t s_tok + h s_head; one with k_scale NULL holds bf16. Keys and values are
  * exact in bf16 (scale included); scores, softmax and sums are fp32, P is rounded to bf16. Unlike echo_attention a
- * row that sees no key gives zeros. `nsplit` > 1 splits the keys over workgroups and joins the parts; it needs
- * echo_attention_fp8_ws_bytes(args, nsplit) bytes of device memory, 16-B aligned. */
+ * row that sees no key gives zeros. The sums of P V are fp32 beside a maximum that may lie 2^8 below the true one:
+ * they are finite wherever 2^8 * keys * max |v| < 2^128. `nsplit` > 1 splits the keys over workgroups and joins the
+ * parts; it needs echo_attention_fp8_ws_bytes(args, nsplit) bytes of device memory, 16-B aligned. */
 typedef struct {
   const void* k; const void* v;
   int64_t ld_tok, ld_batch, ld_head;
