@@ -74,13 +74,14 @@ __device__ __forceinline__ void vm_wait_stages(int n) {
 }
 
 
-// silu(a) * b in fp32: the hardware reciprocal and exp2 (about 2 ulp) are far below the one rounding that follows;
-// for a < -64 (FAR: where one may occur) numerator and divisor are scaled so that the reciprocal stays a normal number
+// silu(a) * b in fp32: the hardware reciprocal and exp2 (about 2 ulp) are far below the one rounding that follows. For
+// a < -64 (FAR: where one may occur) 1 + e^a is 1, and e^a goes to both factors by halves, (a e^(a/2)) (b e^(a/2)): down to
+// a = -174 no half underflows where the product does not
 template <bool FAR = true>
 __device__ __forceinline__ float swiglu_f(float a, float b) {
-  const float sc = FAR && a < -64.0f ? 0x1p-32f : 1.0f;
-  const float d = 1.0f + __builtin_amdgcn_exp2f(a * -1.44269504088896341f);
-  return FAR ? (a * sc) * __builtin_amdgcn_rcpf(d * sc) * b : a * __builtin_amdgcn_rcpf(d) * b;
+  const bool far = FAR && a < -64.0f;
+  const float e = __builtin_amdgcn_exp2f(a * (far ? 0.72134752044448170f : -1.44269504088896341f));
+  return FAR ? (a * (far ? e : __builtin_amdgcn_rcpf(1.0f + e))) * (far ? b * e : b) : a * __builtin_amdgcn_rcpf(1.0f + e) * b;
 }
 
 __device__ __forceinline__ void load4(const bf16_t* p, float (&o)[4]) {

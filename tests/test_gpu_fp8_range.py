@@ -7,6 +7,7 @@ pytestmark = pytest.mark.gpu
 import echo_tts_amd  # noqa: E402,F401
 import fp8_ref as R  # noqa: E402
 import test_gpu_fp8 as T  # noqa: E402
+from echo_tts_amd import _lib as L  # noqa: E402
 from echo_tts_amd import ops  # noqa: E402
 
 DEV, BF, D = "cuda", torch.bfloat16, torch.float64
@@ -47,3 +48,27 @@ def test_attention_large_values(n, nsplit, coded, hot, size):
     ref, tol = T.attention_ref(q, [(kv[:, :, 0], kv[:, :, 1], torch.ones(1, n, lens, dtype=torch.bool, device=DEV))], None, 1.0)
     with ops.attention_split(nsplit):  # beside the long unseen segment more than 32 queries go to the kernel for many
         T.within(ops.attention(q, [seg, T.unseen(1, 1)], scale=1.0), ref, tol)
+
+
+FAR = [-64.0, -64.5, -72.0, -88.0, -89.0, -92.0, -96.0, -100.0, -104.0, -112.0, -130.0, 0.0, 30.0]
+
+
+@pytest.mark.parametrize("M,N", [(13, 32), (13, 512), (160, 1056), (640, 1024), (4100, 1408)])
+def test_swiglu_far(M, N):
+    """silu(a) b with e^a below fp32's range and b = 2^100: a normal number, in bf16 and in 8 bits."""
+    K = 384
+    a = torch.tensor(FAR, dtype=D, device=DEV).repeat(-(-M // len(FAR)))[:M]
+    x = torch.zeros(M, K, dtype=D, device=DEV)
+    x[:, 0] = torch.trunc(a / 8) * 8  # two codes that add up to a, exactly
+    x[:, 1] = a - x[:, 0]
+    x[:, 128] = 2.0 ** 100
+    w = torch.zeros(N, K, dtype=D, device=DEV)
+    w.view(N // 32, 2, 16, K)[:, 0, :, :2] = 1.0
+    w.view(N // 32, 2, 16, K)[:, 1, :, 128] = 1.0
+    (aq, a_s, av), (wq, w_s, wv) = R.matrix(x), R.matrix(w)
+    assert torch.equal(av, x) and torch.equal(wv, w)
+    ref = (a / (1 + torch.exp(-a)) * 2.0 ** 100)[:, None].expand(M, N // 2)
+    err = ref.abs() * ((1.5 * a.abs() + 12) * T.U32)[:, None]  # test_gpu_fp8.swiglu's
+    T.within(ops.gemm_fp8(aq, a_s, wq, w_s, epilogue=L.EPI_SWIGLU), ref, ref.abs() * T.U16 + err * 1.01)
+    q, s = ops.gemm_fp8(aq, a_s, wq, w_s, epilogue=L.EPI_SWIGLU, quantize=True)
+    R.quantized_well(q, R.bytes_of(s, N // 2), ref, 0.0, err * 1.01)
