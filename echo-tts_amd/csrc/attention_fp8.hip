@@ -774,12 +774,19 @@ int64_t items_of(const EchoAttnFp8Args* a) {
   return (int64_t)((a->n_q + qb - 1) / qb) * a->heads * a->rows;
 }
 
+// a grid dimension holds fewer than 2^32 threads; a launch of more is cut without an error
+bool fits(const EchoAttnFp8Args* a, int64_t nsplit) {
+  return items_of(a) <= UINT32_MAX / ((few(a) ? 64 * FW : 256) * max(nsplit, (int64_t)1)) &&
+         (nsplit <= 1 || (int64_t)a->rows * a->heads * 32 * a->n_q <= UINT32_MAX - 255);
+}
+
 bool bad16(const void* p, int64_t bytes) { return (uintptr_t)p % 16 || bytes % 16; }
 
 int check(const EchoAttnFp8Args* a) {
   if (!a) return ECHO_EINVAL;
   if (a->rows < 0 || a->n_q < 0 || a->heads <= 0 || a->nseg < 0 || a->nseg > 4 || a->q_batch_mod < 0) return ECHO_ESHAPE;
   if (a->rows == 0 || a->n_q == 0) return ECHO_OK;
+  if (a->n_q > INT32_MAX - QB || (int64_t)a->rows * a->heads > INT32_MAX) return ECHO_ESHAPE;
   if (!a->q || !a->out || !(a->scale > 0.f)) return ECHO_EINVAL;
   if (bad16(a->q, a->q_ld_tok * 2) || a->q_ld_batch % 8 || bad16(a->out, a->o_ld_tok * 2) || a->o_ld_batch % 8 ||
       (a->gate && (bad16(a->gate, a->g_ld_tok * 2) || a->g_ld_batch % 8)))
@@ -797,7 +804,7 @@ int check(const EchoAttnFp8Args* a) {
     if (g.ld_tok < 0 || g.ld_tok >= (1 << 24) / es || (es == 1 && (g.s_tok < 0 || g.s_tok >= (1 << 24)))) return ECHO_ESHAPE;
     keys += g.capacity;
   }
-  if (keys > INT32_MAX - 256 || items_of(a) > INT32_MAX / 64) return ECHO_ESHAPE;
+  if (keys > INT32_MAX - 256 || !fits(a, 1)) return ECHO_ESHAPE;
   return ECHO_OK;
 }
 
@@ -834,6 +841,7 @@ int echo_attention_fp8(const EchoAttnFp8Args* a, int32_t nsplit, void* ws, int64
   const int rc = check(a);
   if (rc != ECHO_OK || a->rows == 0 || a->n_q == 0) return rc;
   if (nsplit > 64) return ECHO_EINVAL;
+  if (!fits(a, nsplit)) return ECHO_ESHAPE;
   const hipStream_t st = (hipStream_t)stream;
   const int64_t items = items_of(a);
   if (nsplit <= 1) {

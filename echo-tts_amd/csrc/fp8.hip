@@ -22,6 +22,16 @@ __device__ __forceinline__ uint32_t quant8(const float (&x)[8], uint2& codes) {
   return b;
 }
 
+// Waves of a launch, four a workgroup. A grid dimension holds fewer than 2^32 threads (a launch of more is cut without an
+// error), so workgroups from 2^23 on go to a second one.
+__device__ __forceinline__ int64_t wave_of_launch() {
+  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+}
+inline dim3 grid_of(int64_t waves) {
+  const int64_t n = (waves + 3) / 4, x = n < (1 << 23) ? n : 1 << 23;
+  return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
+
 // the four blocks' bytes of a wave as one word (every lane); blocks from `nblk` on are 0
 __device__ __forceinline__ uint32_t scale_word(uint32_t b, int nblk) {
   uint32_t w = 0;
@@ -39,7 +49,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__
                                                            uint32_t* __restrict__ scale, int64_t lds_) {
   const int lane = threadIdx.x & 63;
   const int chunks = (cols + 511) >> 9;
-  const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t task = wave_of_launch();
   if (task >= (int64_t)rows * chunks) return;
   const int row = (int)(task / chunks), c = (int)(task - (int64_t)row * chunks);
   const int col = c * 512 + lane * 8;
@@ -62,8 +72,9 @@ __global__ void __launch_bounds__(256) adaln_fp8_kernel(const T* __restrict__ x,
                                                         uint8_t* __restrict__ q, int64_t ldq,
                                                         uint32_t* __restrict__ scale, int64_t lds_) {
   const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  const int64_t wave = wave_of_launch();
+  if (wave >= rows) return;
+  const int row = (int)wave;
   const T* xr = x + (int64_t)row * dim;
   float v[CH][8];
   float ss = 0.f;
@@ -113,7 +124,7 @@ __global__ void __launch_bounds__(256) kv_write_fp8_kernel(EchoKVWriteArgs a) {
   const int lane = threadIdx.x & 63;
   const int hg = (a.heads + 3) >> 2;
   const int64_t per = (int64_t)a.nblk * 2 * hg;
-  const int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t task = wave_of_launch();
   if (task >= (int64_t)a.batch * a.tokens * per) return;
   const int64_t row = task / per;
   int rest = (int)(task - row * per);
@@ -157,7 +168,6 @@ __global__ void __launch_bounds__(256) kv_write_fp8_kernel(EchoKVWriteArgs a) {
     ((uint8_t*)a.scale)[b * a.s_batch + blk * a.s_blk + kv * a.s_kv + h * a.s_head + slot * a.s_tok] = (uint8_t)byte;
 }
 
-inline unsigned blocks_of(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
 inline bool aligned(const void* p, int64_t ld, int bytes, int a = 16) {
   return (uintptr_t)p % a == 0 && (ld * bytes) % a == 0;
 }
@@ -165,7 +175,7 @@ inline bool aligned(const void* p, int64_t ld, int bytes, int a = 16) {
 template <typename T, int CH>
 void launch_adaln(const void* x, int rows, int dim, const void* shift, const void* scale1, int rpv, int64_t vs, float eps,
                   void* q, int64_t ldq, void* scale, int64_t lds_, hipStream_t st) {
-  hipLaunchKernelGGL((adaln_fp8_kernel<T, CH>), dim3(blocks_of(rows, 4)), dim3(256), 0, st, (const T*)x, rows, dim,
+  hipLaunchKernelGGL((adaln_fp8_kernel<T, CH>), grid_of(rows), dim3(256), 0, st, (const T*)x, rows, dim,
                      (const T*)shift, (const T*)scale1, rpv, vs, eps, (uint8_t*)q, ldq, (uint32_t*)scale, lds_);
 }
 
@@ -192,7 +202,7 @@ int echo_quantize_fp8(int32_t dtype, const void* x, int64_t ldx, int32_t rows, i
   if (!aligned(x, ldx, dtype == ECHO_BF16 ? 2 : 4) || !aligned(q, ldq, 1) || (uintptr_t)scale % 4) return ECHO_EALIGN;
   const int64_t tasks = (int64_t)rows * ((cols + 511) / 512);
   if (tasks > (int64_t)4 * INT32_MAX) return ECHO_ESHAPE;
-  const dim3 grid(blocks_of(tasks, 4));
+  const dim3 grid = grid_of(tasks);
   if (dtype == ECHO_BF16)
     hipLaunchKernelGGL(quantize_fp8_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const bf16_t*)x, ldx, rows,
                        cols, (uint8_t*)q, ldq, (uint32_t*)scale, ld_scale);
@@ -241,7 +251,7 @@ int echo_kv_write_fp8(const EchoKVWriteArgs* a, void* stream) {
     return ECHO_EALIGN;
   const int64_t tasks = (int64_t)a->batch * a->tokens * a->nblk * 2 * ((a->heads + 3) / 4);
   if (tasks > (int64_t)4 * INT32_MAX) return ECHO_ESHAPE;
-  const dim3 grid(blocks_of(tasks, 4));
+  const dim3 grid = grid_of(tasks);
   if (a->dtype == ECHO_BF16)
     hipLaunchKernelGGL(kv_write_fp8_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, *a);
   else

@@ -855,9 +855,13 @@ int ek_of(const EchoGemmFp8Args* a) {
   return a->bias ? EK_BIAS : EK_STORE;
 }
 
+// a grid dimension holds fewer than 2^32 threads; a launch of more is cut without an error
+bool fits(int64_t workgroups, int threads) { return workgroups * threads <= UINT32_MAX; }
+
 template <int BM, int BN, int WM, int WN, int NS>
-void launch_ring(const EchoGemmFp8Args* a, hipStream_t st) {
+int launch_ring(const EchoGemmFp8Args* a, hipStream_t st) {
   const int tm = (a->M + BM - 1) / BM, tn = (a->N + BN - 1) / BN;
+  if (!fits((int64_t)tm * tn, 64 * WM * WN)) return ECHO_ESHAPE;
   const dim3 grid(tm * tn), block(64 * WM * WN);
 #define ECHO_RING(EK) hipLaunchKernelGGL((gemm_fp8_ring_kernel<BM, BN, WM, WN, NS, EK>), grid, block, 0, st, *a, tm, tn)
   if constexpr (BN == 256) {
@@ -872,12 +876,14 @@ void launch_ring(const EchoGemmFp8Args* a, hipStream_t st) {
     }
   }
 #undef ECHO_RING
+  return ECHO_OK;
 }
 
 template <int FM, int FN, int KW, int NS>
-void launch_few(const EchoGemmFp8Args* a, hipStream_t st) {
+int launch_few(const EchoGemmFp8Args* a, hipStream_t st) {
   constexpr int BM = FM * 16, BN = FN * 16;
   const int tm = (a->M + BM - 1) / BM, tn = (a->N + BN - 1) / BN;
+  if (!fits((int64_t)tm * tn, 64 * KW)) return ECHO_ESHAPE;
   const dim3 grid(tm * tn), block(64 * KW);
 #define ECHO_FEW(EK) hipLaunchKernelGGL((gemm_fp8_few_kernel<FM, FN, KW, NS, EK>), grid, block, 0, st, *a, tm, tn)
   switch (ek_of(a)) {
@@ -888,9 +894,10 @@ void launch_few(const EchoGemmFp8Args* a, hipStream_t st) {
     default: if constexpr (FN > 1) ECHO_FEW(EK_SWIGLU);
   }
 #undef ECHO_FEW
+  return ECHO_OK;
 }
 
-void launch_ps(const EchoGemmFp8Args* a, hipStream_t st) {
+int launch_ps(const EchoGemmFp8Args* a, hipStream_t st) {
   const int tm = (a->M + 255) / 256, tn = (a->N + 255) / 256;
   const dim3 grid(min(tm * tn, cu_count())), block(256);
 #define ECHO_PS(EK) hipLaunchKernelGGL(gemm_fp8_ps_kernel<EK>, grid, block, 0, st, *a, tm, tn, 4)
@@ -903,6 +910,7 @@ void launch_ps(const EchoGemmFp8Args* a, hipStream_t st) {
     default: ECHO_PS(EK_SWIGLU_Q);
   }
 #undef ECHO_PS
+  return ECHO_OK;
 }
 
 // The kernels, and what a launch of each costs: rounds of workgroups over the chip (256 CUs) x (1.1 us + K-tiles x the time
@@ -953,7 +961,7 @@ int check(const EchoGemmFp8Args* a) {
   if (glu && (a->bias || a->aux || a->gate)) return ECHO_EINVAL;
   if (a->epilogue == ECHO_EPI_STORE && (a->aux || a->gate)) return ECHO_EINVAL;
   const int nout = glu ? a->N / 2 : a->N;
-  if (a->M < 0 || a->N <= 0 || a->K <= 0 || a->K % 16 || a->N % (glu ? 32 : 16)) return ECHO_ESHAPE;
+  if (a->M < 0 || a->M > INT32_MAX - 255 || a->N <= 0 || a->K <= 0 || a->K % 16 || a->N % (glu ? 32 : 16)) return ECHO_ESHAPE;
   // 32-bit byte offsets inside a tile of up to 256 rows
   if (a->lda < a->K || a->ldw < a->K || a->ldc < nout || a->lda > (1 << 22) || a->ldw > (1 << 22) ||
       a->ldc > (1 << 21)) return ECHO_ESHAPE;
@@ -975,21 +983,22 @@ int check(const EchoGemmFp8Args* a) {
 extern "C" {
 
 int echo_gemm_fp8(const EchoGemmFp8Args* a, void* stream) {
-  const int rc = check(a);
+  int rc = check(a);
   if (rc != ECHO_OK || a->M == 0) return rc;
   const hipStream_t st = (hipStream_t)stream;
   switch (pick(a)) {
-    case FEW_16x16: launch_few<1, 1, 8, 4>(a, st); break;
-    case FEW_16x32: launch_few<1, 2, 8, 3>(a, st); break;
-    case FEW_32x32: launch_few<2, 2, 4, 4>(a, st); break;
-    case FEW_64x32: launch_few<4, 2, 4, 3>(a, st); break;
-    case FEW_64x64: launch_few<4, 4, 4, 2>(a, st); break;
-    case RING_64: launch_ring<64, 64, 2, 2, 4>(a, st); break;
-    case RING_128: launch_ring<128, 128, 4, 2, 3>(a, st); break;
-    case RING_32_Q: launch_ring<32, 256, 1, 4, 3>(a, st); break;
-    case RING_64_Q: launch_ring<64, 256, 2, 4, 3>(a, st); break;
-    case PS: launch_ps(a, st); break;
+    case FEW_16x16: rc = launch_few<1, 1, 8, 4>(a, st); break;
+    case FEW_16x32: rc = launch_few<1, 2, 8, 3>(a, st); break;
+    case FEW_32x32: rc = launch_few<2, 2, 4, 4>(a, st); break;
+    case FEW_64x32: rc = launch_few<4, 2, 4, 3>(a, st); break;
+    case FEW_64x64: rc = launch_few<4, 4, 4, 2>(a, st); break;
+    case RING_64: rc = launch_ring<64, 64, 2, 2, 4>(a, st); break;
+    case RING_128: rc = launch_ring<128, 128, 4, 2, 3>(a, st); break;
+    case RING_32_Q: rc = launch_ring<32, 256, 1, 4, 3>(a, st); break;
+    case RING_64_Q: rc = launch_ring<64, 256, 2, 4, 3>(a, st); break;
+    case PS: rc = launch_ps(a, st); break;
   }
+  if (rc != ECHO_OK) return rc;
   ECHO_LAUNCH_CHECK();
   return ECHO_OK;
 }

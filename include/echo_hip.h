@@ -389,7 +389,8 @@ int echo_kv_write_fp8(const EchoKVWriteArgs* args, void* stream);
  *   ECHO_EPI_RESID:  aux[m][n] + gate[n] * (acc (+ bias[n]))      (gate NULL: 1; aux may be C itself)
  *   ECHO_EPI_SWIGLU: silu(a) * b of W rows interleaved in blocks of 16 as in echo_gemm; C has N / 2 columns
  * C, bias, aux, gate are bf16; c_scale != NULL (ECHO_EPI_SWIGLU only): C is e4m3 codes and c_scale their scales.
- * K % 16 == 0, N % 16 == 0 (SWIGLU: N % 32 == 0), any M; lda, ldw <= 2^22, ldc, ld_aux <= 2^21. */
+ * K % 16 == 0, N % 16 == 0 (SWIGLU: N % 32 == 0), any M; lda, ldw <= 2^22, ldc, ld_aux <= 2^21. An output whose
+ * launch would need 2^32 threads is refused with ECHO_ESHAPE. */
 typedef struct {
   int32_t M, N, K, epilogue;
   const void* A; int64_t lda; const void* a_scale; int64_t ld_as;
@@ -407,7 +408,8 @@ int echo_gemm_fp8(const EchoGemmFp8Args* args, void* stream);
  * exact in bf16 (scale included); scores, softmax and sums are fp32, P is rounded to bf16. Unlike echo_attention a
  * row that sees no key gives zeros. The sums of P V are fp32 beside a maximum that may lie 2^8 below the true one:
  * they are finite wherever 2^8 * keys * max |v| < 2^128. `nsplit` > 1 splits the keys over workgroups and joins the
- * parts; it needs echo_attention_fp8_ws_bytes(args, nsplit) bytes of device memory, 16-B aligned. */
+ * parts; it needs echo_attention_fp8_ws_bytes(args, nsplit) bytes of device memory, 16-B aligned. Launches of 2^32 threads
+ * (rows * heads * nsplit >= 2^23 for up to 32 queries) are refused with ECHO_ESHAPE. */
 typedef struct {
   const void* k; const void* v;
   int64_t ld_tok, ld_batch, ld_head;
