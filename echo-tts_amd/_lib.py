@@ -140,6 +140,7 @@ SIGNATURES = {
     "echo_adaln_modulate_fp8": (i32, [i32, vp, i32, i32, vp, vp, i32, i64, f32, vp, i64, vp, i64, vp]),
     "echo_kv_write_fp8": (i32, [C.POINTER(KVWriteArgs), vp]),
     "echo_gemm_fp8": (i32, [C.POINTER(GemmFp8Args), vp]),
+    "echo_gemm_fp8_planned_kernel": (i32, [C.POINTER(GemmFp8Args)]),
     "echo_attention_fp8_pick_split": (i32, [C.POINTER(AttnFp8Args)]),
     "echo_attention_fp8_ws_bytes": (i64, [C.POINTER(AttnFp8Args), i32]),
     "echo_attention_fp8": (i32, [C.POINTER(AttnFp8Args), i32, vp, i64, vp]),

@@ -982,6 +982,11 @@ int check(const EchoGemmFp8Args* a) {
 
 extern "C" {
 
+int32_t echo_gemm_fp8_planned_kernel(const EchoGemmFp8Args* a) {
+  const int rc = check(a);
+  return rc != ECHO_OK ? rc : a->M == 0 ? PS + 1 : pick(a);
+}
+
 int echo_gemm_fp8(const EchoGemmFp8Args* a, void* stream) {
   int rc = check(a);
   if (rc != ECHO_OK || a->M == 0) return rc;

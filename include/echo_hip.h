@@ -401,6 +401,10 @@ typedef struct {
   const void* gate;
 } EchoGemmFp8Args;
 int echo_gemm_fp8(const EchoGemmFp8Args* args, void* stream);
+/* Host-only query: the kernel of echo_gemm_fp8(args, .) (the routine that decides both). Tiles of M x N: 0 to 4 = 16x16,
+ * 16x32, 32x32, 64x32, 64x64 whose waves share K; 5, 6 = 64x64, 128x128 LDS rings; 7, 8 = 32x256, 64x256 rings (8-bit
+ * output); 9 = persistent 256x256; 10 = none (M == 0); negative: the error. */
+int32_t echo_gemm_fp8_planned_kernel(const EchoGemmFp8Args* args);
 
 /* echo_attention over segments that may be 8-bit caches: bf16 q, gate and out; a segment with k_scale != NULL holds
  * e4m3 codes in blocks of one head's 128 (head h of token t at k + b ld_batch + t ld_tok + h ld_head, in elements)
