@@ -72,3 +72,23 @@ def test_swiglu_far(M, N):
     T.within(ops.gemm_fp8(aq, a_s, wq, w_s, epilogue=L.EPI_SWIGLU), ref, ref.abs() * T.U16 + err * 1.01)
     q, s = ops.gemm_fp8(aq, a_s, wq, w_s, epilogue=L.EPI_SWIGLU, quantize=True)
     R.quantized_well(q, R.bytes_of(s, N // 2), ref, 0.0, err * 1.01)
+
+
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_attention_small_values(n):
+    """Blocks below 2^-118 keep the smallest scale, 2^-127 (byte 0): values of 2^-120 come back, and keys alike."""
+    lens = 200
+    kv = torch.randn(1, lens, 2, 1, 128, device=DEV) * 2.0 ** -120
+    c, b = R.quantize(kv)
+    assert int(b.max()) <= 2 and int(b.min()) == 0
+    cache, scale = T.new_cache(1, lens, 1, 1, "plain")
+    cache.view(torch.uint8)[:, :, 0] = c.view(torch.uint8)
+    scale.view(torch.uint8)[:, 0] = b[..., 0].permute(0, 2, 3, 1)
+    kv = R.values(c, b)
+    q = torch.randn(1, n, 1, 128, device=DEV).to(BF) * 2.0 ** 118  # scores of a few units
+    ref, tol = T.attention_ref(q, [(kv[:, :, 0], kv[:, :, 1], torch.ones(1, n, lens, dtype=torch.bool, device=DEV))], None)
+    # attention_ref's tolerance has 1e-30 beside the relative part: here in units of 2^120
+    e = (tol - 1e-30) * 2.0 ** 120
+    for segs in ([T.segment(cache, scale)], [T.segment(cache, scale), T.unseen(1, 1)]):
+        out = ops.attention(q, segs)
+        T.within(out.to(D) * 2.0 ** 120, ref * 2.0 ** 120, e + 2.0 ** -13)  # 2^-133: bf16's last subnormal bit
