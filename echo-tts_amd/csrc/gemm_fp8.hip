@@ -74,12 +74,14 @@ __device__ __forceinline__ void vm_wait_stages(int n) {
 }
 
 
-// silu(a) * b in fp32: the hardware reciprocal and exp2 (about 2 ulp) are far below the one rounding that follows. For
-// a < -64 (FAR: where one may occur) 1 + e^a is 1, and e^a goes to both factors by halves, (a e^(a/2)) (b e^(a/2)): down to
-// a = -174 no half underflows where the product does not
+// silu(a) * b in fp32: the hardware reciprocal and exp2 (about 2 ulp) are far below the one rounding that follows. From
+// a = -87 on down (FAR: where one may occur) the reciprocal of 1 + e^-a would leave the normal numbers; there 1 + e^a is 1,
+// and e^a goes to both factors by halves, (a e^(a/2)) (b e^(a/2)): down to a = -174 no half underflows where the product
+// does not
+constexpr float SILU_FAR = -87.0f;
 template <bool FAR = true>
 __device__ __forceinline__ float swiglu_f(float a, float b) {
-  const bool far = FAR && a < -64.0f;
+  const bool far = FAR && a < SILU_FAR;
   const float e = __builtin_amdgcn_exp2f(a * (far ? 0.72134752044448170f : -1.44269504088896341f));
   return FAR ? (a * (far ? e : __builtin_amdgcn_rcpf(1.0f + e))) * (far ? b * e : b) : a * __builtin_amdgcn_rcpf(1.0f + e) * b;
 }
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(256, 1) gemm_fp8_ps_kernel(EchoGemmFp8Args a, 
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 8; ++e) lo = fminf(lo, acc[i][j][e]);
-        if (__builtin_expect(__any(!(lo >= -64.0f)), 0)) {
+        if (__builtin_expect(__any(!(lo >= SILU_FAR)), 0)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll

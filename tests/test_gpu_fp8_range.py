@@ -53,11 +53,24 @@ def test_attention_large_values(n, nsplit, coded, hot, size):
 FAR = [-64.0, -64.5, -72.0, -88.0, -89.0, -92.0, -96.0, -100.0, -104.0, -112.0, -130.0, 0.0, 30.0]
 
 
-@pytest.mark.parametrize("M,N", [(13, 32), (13, 512), (160, 1056), (640, 1024), (4100, 1408)])
+SHAPES = [(13, 32), (13, 512), (160, 1056), (640, 1024), (4100, 1408)]
+
+
+@pytest.mark.parametrize("M,N", SHAPES)
 def test_swiglu_far(M, N):
     """silu(a) b with e^a below fp32's range and b = 2^100: a normal number, in bf16 and in 8 bits."""
+    swiglu_of(FAR, M, N)
+
+
+@pytest.mark.parametrize("M,N", SHAPES)
+def test_swiglu_border(M, N):
+    """Around a = -87, below which the reciprocal of 1 + e^-a is no normal number."""
+    swiglu_of([-86.0, -86.5, -87.0, -87.5, -88.0], M, N)
+
+
+def swiglu_of(values, M, N):
     K = 384
-    a = torch.tensor(FAR, dtype=D, device=DEV).repeat(-(-M // len(FAR)))[:M]
+    a = torch.tensor(values, dtype=D, device=DEV).repeat(-(-M // len(values)))[:M]
     x = torch.zeros(M, K, dtype=D, device=DEV)
     x[:, 0] = torch.trunc(a / 8) * 8  # two codes that add up to a, exactly
     x[:, 1] = a - x[:, 0]
