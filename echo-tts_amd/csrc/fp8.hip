@@ -23,12 +23,13 @@ __device__ __forceinline__ uint32_t quant8(const float (&x)[8], uint2& codes) {
 }
 
 // Waves of a launch, four a workgroup. A grid dimension holds fewer than 2^32 threads (a launch of more is cut without an
-// error), so workgroups from 2^23 on go to a second one.
+// error), so from 2^23 workgroups on they go to a second one.
+constexpr int GRID_X = 23;
 __device__ __forceinline__ int64_t wave_of_launch() {
-  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  return (((int64_t)blockIdx.y << GRID_X) + blockIdx.x) * 4 + (threadIdx.x >> 6);
 }
 inline dim3 grid_of(int64_t waves) {
-  const int64_t n = (waves + 3) / 4, x = n < (1 << 23) ? n : 1 << 23;
+  const int64_t n = (waves + 3) / 4, x = min(n, (int64_t)1 << GRID_X);
   return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
 }
 
