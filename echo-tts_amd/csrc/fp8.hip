@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t scale_word(uint32_t b, int nblk) {
 }
 
 // One wave per 512-column chunk (four blocks) of a row: no wave depends on another, so small matrices spread over the chip.
-// 30720 x 2048 bf16: 32-36 us, 5.3 TB/s (a copy's rate 4.9); 157 x 1360 fp32: 2.6 us.
+// 30720 x 2048 bf16: the kernel 32 us (5.9 TB/s), a call among others 36 (5.2; a copy's rate 4.9); 157 x 1360 fp32: 2.6 us.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols,
                                                            uint8_t* __restrict__ q, int64_t ldq,
@@ -64,8 +64,9 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__
 }
 
 // y = (x * rsqrt(mean x^2 + eps)) * scale1 + shift in fp32, quantised: one wave per row, the row in registers, so that x is
-// read once. CH: 512-column chunks held (2, 4, 8, 16 by dim). 30720 x 2048 bf16: 43 us, 4.4 TB/s; 640 x 2048: 5.0 us, the
-// latencies of a row's loads, its sum and the vectors' loads one after the other.
+// read once. CH: 512-column chunks held (2, 4, 8, 16 by dim). 30720 x 2048 bf16: the kernel 36 us (5.3 TB/s), a call
+// among others 43 (4.4); 640 x 2048: 5.1 us, the latencies of a row's loads, its sum and the vectors' loads one after the other.
+// Codes that differ from those of the 64-bit value: 62 to 77 of 63 million (as many as for torch's fp32 operations).
 template <typename T, int CH>
 __global__ void __launch_bounds__(256) adaln_fp8_kernel(const T* __restrict__ x, int rows, int dim,
                                                         const T* __restrict__ shift, const T* __restrict__ scale1,
@@ -117,9 +118,10 @@ __global__ void __launch_bounds__(256) adaln_fp8_kernel(const T* __restrict__ x,
 // Token t of sequence b goes to slot start[b] + t (start NULL: t) if t < lens[b] and the slot lies in the cache; every
 // other slot keeps its bytes. Keys get the head RMS norm (w) and interleaved rotary pairs on heads < rope_heads, at
 // position pos0 + pos_mult * slot; fp32 throughout, the only rounding is the code's.
-// 2 x 1600 tokens (0.56 of them valid), 24 layers, 16 heads, bf16: 145-180 us, 3.0-3.7 TB/s; 4 x 1: 2.8 us. Consecutive
-// waves take consecutive bytes of x. Tokens in groups (2 to 16, so that their scale bytes, which lie beside each other, are
-// written together) took 186 us, and an XCD's own range of tokens 250 us.
+// 2 x 1600 tokens (1800 of them valid), 24 layers, 16 heads, bf16: 182 us, 2.9 TB/s: the scale bytes of a
+// token lie a capacity apart. 4 x 1: 3.5 us. Consecutive waves take consecutive bytes of x. Tokens in groups (2 to 16, so
+// that their scale bytes, which lie beside each other, are written together) took 186 us, and an XCD's own range of tokens
+// 250 us.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_write_fp8_kernel(EchoKVWriteArgs a) {
   const int lane = threadIdx.x & 63;

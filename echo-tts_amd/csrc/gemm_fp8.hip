@@ -399,7 +399,8 @@ gemm_fp8_few_kernel(EchoGemmFp8Args a, int tiles_m, int tiles_n) {
 // so two LDS slots of a block do: what a step requests goes where everything was read a step before, and has two to three
 // steps to land. A DMA instruction takes 8 whole rows of 128 B: at 64 B a row (steps of half a block, four slots) L2 serves
 // one request a clock and channel at half width and was the bound (30720x8192x2048: 485 us, 66 % of the cycles in MFMA;
-// now 423-435 us, 2.4 PFLOP/s at the clock that the card's power limit leaves; 30720x11776x2048 SwiGLU in 8 bits 592-614).
+// now 424 us on one input, 436 on new inputs each time, 2.4 PFLOP/s at the clock that the card's power limit leaves;
+// 30720x11776x2048 SwiGLU to 8 bits 604 and 630).
 // One barrier a step: at its start every wave has its fragments in registers and everybody's share of what the step reads
 // has landed (vmcnt counts in issue order: 16 younger operations stay in flight, whichever step it is).
 // After a tile's last step the next tile's two blocks are requested before the epilogue, which works from the

@@ -405,7 +405,9 @@ def adaln_modulate_fp8(x: Tensor, shift: Tensor, scale1: Tensor, eps: float,
 def gemm_fp8(a: Tensor, a_scale: Tensor, w: Tensor, w_scale: Tensor, out: Optional[Tensor] = None, *,
              bias: Optional[Tensor] = None, epilogue: int = L.EPI_STORE, aux: Optional[Tensor] = None,
              gate: Optional[Tensor] = None, quantize: bool = False, out_scale: Optional[Tensor] = None):
-    """a [M, K] @ w [N, K]^T of two matrices in the 8-bit format, fp32 accumulation, bfloat16 out (one rounding).
+    """a [M, K] @ w [N, K]^T of two matrices in the 8-bit format, bfloat16 out (one rounding). Sums are fp32 above groups
+    of 8 consecutive k, whose products the matrix instruction cuts to 2^-13 of the largest one (2^-18 of sum |a w| on
+    random inputs): of the codes of a quantised output 0.25 to 0.4 % lie a step beside those of the exact product.
 
     epilogue: EPI_STORE (+ bias [N]); EPI_RESID out = aux + gate * (acc + bias), aux may be out; EPI_SWIGLU of W rows
     interleaved in blocks of 16 (N / 2 columns). quantize (EPI_SWIGLU): the output in the 8-bit format, (codes, scale);

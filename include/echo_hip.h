@@ -384,7 +384,9 @@ typedef struct {
 } EchoKVWriteArgs;
 int echo_kv_write_fp8(const EchoKVWriteArgs* args, void* stream);
 
-/* C = tail(A . W^T) with A [M, K] and W [N, K] in the 8-bit format, fp32 accumulation, one rounding at the end:
+/* C = tail(A . W^T) with A [M, K] and W [N, K] in the 8-bit format, one rounding at the end. Sums are fp32 above groups of 8
+ * consecutive k, whose products the matrix instruction cuts to 2^-13 of the largest one (2^-18 of sum |a w| on random
+ * inputs):
  *   ECHO_EPI_STORE:  acc (+ bias[n])
  *   ECHO_EPI_RESID:  aux[m][n] + gate[n] * (acc (+ bias[n]))      (gate NULL: 1; aux may be C itself)
  *   ECHO_EPI_SWIGLU: silu(a) * b of W rows interleaved in blocks of 16 as in echo_gemm; C has N / 2 columns
