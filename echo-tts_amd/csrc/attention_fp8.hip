@@ -6,10 +6,10 @@
 // 32 queries of one (row, head), 64-key tiles, scores transposed (S^T = K Q^T, v_mfma_f32_32x32x16_bf16) so that a lane
 // holds one query's keys, maximum and sum in fp32, P in bf16 straight from the accumulators into O^T += V^T P.
 // What bounds it: 48 rows x 640 queries x 16 heads, half of the ~1350 keys a query own (bf16), half cached: 486-516 us, 750
-// TFLOP/s. Under counters (545-595 us, 1.65-1.8 GHz) a SIMD's 983k cycles are 360k MFMA and 521k vector (exp2, conversion of
-// codes, sums), of which two waves overlap little: all-bf16 keys in attention.hip's kernel take 437 us. Measured against it, 8 waves in two groups a phase apart (one in its
-// MFMAs while the other converts and exponentiates, swapped by barriers): 590 us, though 3 rows of 640 queries take 58
-// instead of 68 us; fragments read 5 MFMAs ahead: 528 us.
+// TFLOP/s (with bf16 caches attention.hip's kernel takes 437). Under counters (545-595 us, 1.65-1.8 GHz) a SIMD's 983k cycles
+// are 360k MFMA and 521k vector (exp2, conversion of codes, sums), of which two waves overlap little. Measured against it, 8
+// waves in two groups a phase apart (one in its MFMAs while the other converts and exponentiates, swapped by barriers): 590
+// us, though 3 rows of 640 queries take 58 instead of 68 us; fragments read 5 MFMAs ahead: 528 us.
 #include "fp8.h"
 
 #include <type_traits>
